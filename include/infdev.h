@@ -295,7 +295,9 @@ int infdev_mtp_fuse(infdev_ctx* ctx, const float* embedding, const float* hidden
  * repetition must be positive. A row whose mask allows nothing comes out as -infinity throughout. Token ids outside the vocabulary, in the history or with a bias, count for nothing. */
 int infdev_adjust_logits(infdev_ctx* ctx, const float* logits, int64_t vocab, const infdev_query* queries, int queryCount, int64_t count,
                          const infdev_logit_rules* rules, const int32_t* tokens, uint32_t capacity, const int32_t* proposals, float* out);
-/* sample_logits (native_ops.metal:122-224): logits fp32 [count,vocab]; mode 0 target, 1 MTP drafting. */
+/* sample_logits (native_ops.metal:122-224): logits fp32 [count,vocab]; mode 0 target, 1 MTP drafting. A token whose logit is -infinity or not a number is
+ * not drawn while another is above -infinity, and one of +infinity always is. A row without any above -infinity (a mask that allows nothing) is not reported: its token is 0, or
+ * vocab - 1 with a temperature and topK 0. */
 int infdev_sample(infdev_ctx* ctx, const float* logits, int64_t vocab, infdev_query* queries, int queryCount, int64_t count, uint32_t mode,
                   int32_t* tokens);
 /* The packing loop of forward() (forward.cpp:171-191) on the device. in[i].samples carries the slot's

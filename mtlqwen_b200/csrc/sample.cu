@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     // double precision in contiguous chunks, 128 of them per CTA and two at a time per warp; the first CTA finds the chunk
     // in which the cumulative sum passes the target and walks that one in vocabulary order. What bounds it is latency, so everything is
     // asked for eight values at a time: one and eight rows of 248320 logits 33.4 -> 17.0 and 37.5 -> 20.5 us, in the order of addition as before.
-    maximum = fmaxf(fmaxf(sh.maxima[lane], sh.maxima[lane + 32]), fmaxf(sh.maxima[lane + 64], sh.maxima[lane + 96]));
-    maximum = warp_max(maximum) / temperature;
+    const float most = warp_max(fmaxf(fmaxf(sh.maxima[lane], sh.maxima[lane + 32]), fmaxf(sh.maxima[lane + 64], sh.maxima[lane + 96])));
+    maximum = most / temperature;
     const int chunks = int(ctas) * kChunks, chunk = (vocab + chunks - 1) / chunks;
     for (int c = int(part) * kChunks + warp; c < int(part + 1) * kChunks; c += 2 * kClusterWarps) {
       double sum[2] = {0.0, 0.0};  // of two chunks at a time
@@ -297,9 +297,31 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
       if (lane >= o)
         inclusive += other;
     }
-    const double target = double(random) * __shfl_sync(0xffffffffu, inclusive, 31);
-    const uint32_t reached = __ballot_sync(0xffffffffu, inclusive >= target);
-    const int ownerLane = reached ? __ffs(reached) - 1 : 31;
+    const double total = __shfl_sync(0xffffffffu, inclusive, 31), target = double(random) * total;
+    // Infinite quotients, or logits that are not numbers, leave no sum to draw from: the first of the largest logits. (The last token of a row without a logit above -infinity.)
+    if (!(total > 0.0)) {
+      int token = vocab - 1;
+      for (int base = 0; base < vocab && most > -INFINITY; base += 8 * kWarp) {
+        uint32_t equal = 0;  // bit e: the logit kWarp e further on
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (base + kWarp * e + lane < vocab && row[base + kWarp * e + lane] == most)
+            equal |= 1u << e;
+        const int here = equal ? kWarp * (__ffs(equal) - 1) + lane : 8 * kWarp, least = __reduce_min_sync(0xffffffffu, here);
+        if (least < 8 * kWarp) {
+          token = base + least;
+          break;
+        }
+      }
+      if (lane == 0)
+        tokens[i] = token;
+      return;
+    }
+    // Only what has a weight is drawn, of lanes, chunks and tokens: a target of 0 is reached where nothing has been added yet, and sums that were added up in another order
+    // may reach the target a rounding earlier or not at all, which is then the last one's.
+    const bool some = lanes32 > 0.0;
+    const uint32_t reached = __ballot_sync(0xffffffffu, some && inclusive >= target), any = __ballot_sync(0xffffffffu, some);
+    const int ownerLane = reached ? __ffs(reached) - 1 : 31 - __clz(any);
     if (lane == ownerLane) {
       double cumulative = inclusive - lanes32;
       int owner = lane * perLane;
@@ -312,17 +334,19 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         const int at = owner;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          before = before && at + e < end && cumulative + sums[e] < target;
+          before = before && at + e < end && !(sums[e] > 0.0 && cumulative + sums[e] >= target);
           if (before)
             cumulative += sums[e], ++owner;
         }
       }
+      while (!(sh.chunkSum[owner] > 0.0))  // the last chunk; one before it has a weight
+        cumulative -= sh.chunkSum[--owner];
       sh.owner = owner, sh.before = cumulative;
     }
     __syncwarp();
     double cumulative = sh.before;
     const int a = sh.owner * chunk, b = min(vocab, a + chunk);
-    int token = vocab - 1;
+    int token = -1;
     float value[8];
     for (int base = a, e = 0; base < b; base += 32, ++e) {
       const int j = base + lane;
@@ -330,7 +354,8 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
 #pragma unroll
         for (int ahead = 0; ahead < 8; ++ahead)
           value[ahead] = j + 32 * ahead < b ? row[j + 32 * ahead] : 0.f;
-      double running = j < b ? double(expf(value[0] / temperature - maximum)) : 0.0;
+      const double weight = j < b ? double(expf(value[0] / temperature - maximum)) : 0.0;
+      double running = weight;
 #pragma unroll
       for (int ahead = 0; ahead < 7; ++ahead)
         value[ahead] = value[ahead + 1];
@@ -340,12 +365,17 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         if (lane >= o)
           running += other;
       }
-      const uint32_t hit = __ballot_sync(0xffffffffu, j < b && cumulative + running >= target);
+      const uint32_t hit = __ballot_sync(0xffffffffu, weight > 0.0 && cumulative + running >= target);
       if (hit) {
         token = base + __ffs(hit) - 1;
         break;
       }
       cumulative += __shfl_sync(0xffffffffu, running, 31);
+    }
+    for (int base = (b - 1 - a) / kWarp * kWarp + a; token < 0 && base >= a; base -= kWarp) {
+      const uint32_t weighs = __ballot_sync(0xffffffffu, base + lane < b && expf(row[base + lane] / temperature - maximum) > 0.f);
+      if (weighs)
+        token = base + 31 - __clz(weighs);
     }
     if (lane == 0)
       tokens[i] = token;

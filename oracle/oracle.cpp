@@ -474,7 +474,8 @@ float orc_uniform(uint64_t key, uint64_t counter) {
 // top_k > 0: the min(top_k,64) largest logits/temperature in descending order, ties by ascending index
 // (the insertion sort of :194-207 is stable and skips equal values), top-p inside that set (:208-215),
 // inverse-CDF pick with `random` (:216-223). top_k == 0: plain temperature sampling over the vocabulary,
-// top-p ignored (:172-188). `margin` (nullable) receives best - second best logit for greedy rows.
+// top-p ignored (:172-188); a token without a weight (a masked one) is never drawn, as the reference's first one is by a variate of 0, and
+// where the weights have no sum (infinite logits, or none that is a number) the first of the largest logits is. `margin` (nullable) receives best - second best logit for greedy rows.
 int32_t orc_sample(const float* logits, int64_t vocab, float temperature, float topP, int32_t topK, float random, float* margin) {
   if (temperature <= 0) {
     int64_t best = 0;
@@ -496,13 +497,27 @@ int32_t orc_sample(const float* logits, int64_t vocab, float temperature, float 
     double total = 0.0;
     for (int64_t j = 0; j < vocab; ++j)
       total += double(std::exp(logits[j] / temperature - maximum));
+    int64_t last = vocab - 1;
+    if (!(total > 0)) {
+      float most = -INFINITY;
+      for (int64_t j = 0; j < vocab; ++j)
+        if (logits[j] > most) {
+          most = logits[j];
+          last = j;
+        }
+      return int32_t(last);
+    }
     double target = double(random) * total, cumulative = 0.0;
     for (int64_t j = 0; j < vocab; ++j) {
-      cumulative += double(std::exp(logits[j] / temperature - maximum));
+      double weight = double(std::exp(logits[j] / temperature - maximum));
+      if (!(weight > 0))
+        continue;
+      cumulative += weight;
+      last = j;
       if (cumulative >= target)
-        return int32_t(j);
+        break;
     }
-    return int32_t(vocab - 1);
+    return int32_t(last);
   }
   float values[64];
   int64_t indices[64];
