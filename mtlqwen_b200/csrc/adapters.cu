@@ -628,7 +628,8 @@ template <class W> struct OuterShared {
   __align__(16) uint8_t weights[kOuterWarps][2][kUnit * kStagePitch];
   __align__(16) uint32_t inner[Format<W>::kPieces][kInner / 2];  // inner products, scaled and cut: [piece][tile of 16 ranks][row][pair of ranks], pairs in the order 0 4 1 5 2 6 3 7
   __align__(16) float uncut[Format<W>::kHalf ? kInner : 4];      // fp16: before they are cut
-  uint32_t largest[32];                                          // fp16: of a row of them, the bits of its magnitude
+  uint32_t largest[2][32];                                       // fp16: of a row of them and a matrix of a pair, the bits of its magnitude
+  __align__(8) float back[2][32];                                // fp16: what brings their products back to scale
   int rows[32];
 };
 static_assert(2 * kAdapterMaxRank * 8 <= kInner, "eight rows of a pair of the largest ranks fit");
@@ -793,8 +794,8 @@ __device__ __forceinline__ void run_units(const AdapterParams& p, OuterShared<W>
   // ---- the inner products: the sum of their parts, scaled and cut
   const int values = tiles * kRows * 16;
   if (kHalf) {
-    if (tid < kRows)
-      sh.largest[tid] = 0;
+    if (tid < kHalves * kRows)
+      sh.largest[tid / kRows][tid % kRows] = 0;
     __syncthreads();
   }
   auto cut = [&](int i, float4 v) {
@@ -838,7 +839,7 @@ __device__ __forceinline__ void run_units(const AdapterParams& p, OuterShared<W>
         v[e] = e < left[k] ? v[e] * scale[k] : 0.f;
       if constexpr (kHalf) {
         *reinterpret_cast<float4*>(sh.uncut + i) = make_float4(v[0], v[1], v[2], v[3]);
-        atomicMax(&sh.largest[i / 16 % kRows], __float_as_uint(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])))));
+        atomicMax(&sh.largest[PAIR && i >= tiles0 * kRows * 16][i / 16 % kRows], __float_as_uint(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])))));
       } else {
         cut(i, make_float4(v[0], v[1], v[2], v[3]));
       }
@@ -846,25 +847,19 @@ __device__ __forceinline__ void run_units(const AdapterParams& p, OuterShared<W>
   }
   if constexpr (kHalf) {
     __syncthreads();
+    if (tid < kHalves * kRows) {
+      float to;
+      range_of(__uint_as_float(sh.largest[tid / kRows][tid % kRows]), to, sh.back[tid / kRows][tid % kRows]);
+    }
 #pragma unroll 1
     for (int i = tid * 4; i < values; i += kThreads * 4) {
       float to, back;
-      range_of(__uint_as_float(sh.largest[i / 16 % kRows]), to, back);
+      range_of(__uint_as_float(sh.largest[PAIR && i >= tiles0 * kRows * 16][i / 16 % kRows]), to, back);
       const float4 v = *reinterpret_cast<const float4*>(sh.uncut + i);
       cut(i, make_float4(v.x * to, v.y * to, v.z * to, v.w * to));
     }
   }
   __syncthreads();  // the inner products are there
-  float back[NT][2];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float to;
-      back[j][e] = 1.f;
-      if (kHalf)
-        range_of(__uint_as_float(sh.largest[8 * j + 2 * t + e]), to, back[j][e]);
-    }
   // ---- columns
   int stage = 0;
 #pragma unroll 1
@@ -901,16 +896,21 @@ __device__ __forceinline__ void run_units(const AdapterParams& p, OuterShared<W>
       if (8 * j >= live)
         break;
       const float2(&rows)[kHalves][2] = held[j];
+      float2 back[kHalves];  // of both rows
+#pragma unroll
+      for (int half = 0; half < kHalves; ++half)
+        back[half] = kHalf ? *reinterpret_cast<const float2*>(&sh.back[half][8 * j + 2 * t]) : make_float2(1.f, 1.f);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         if (8 * j + e >= live)
           break;
-        const float unitOf = back[j][e];
+        const float unitOf = e ? back[0].y : back[0].x;
         float2 v = rows[0][e];
         v.x += d[0][j][e] * unitOf, v.y += d[0][j][2 + e] * unitOf;
         if constexpr (PAIR) {
           const float2 u = rows[1][e];
-          v.x = silu_f(v.x) * (u.x + d[1][j][e] * unitOf), v.y = silu_f(v.y) * (u.y + d[1][j][2 + e] * unitOf);
+          const float upOf = e ? back[1].y : back[1].x;
+          v.x = silu_f(v.x) * (u.x + d[1][j][e] * upOf), v.y = silu_f(v.y) * (u.y + d[1][j][2 + e] * upOf);
         }
         if (8 * j + 2 * t + e < live && column < n)
           store_columns<VEC>(y + (rowAt[j][e] + column), v, n - column);
