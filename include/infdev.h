@@ -187,7 +187,8 @@ int infdev_gate_up(infdev_ctx* ctx, int type, const void* wg, const void* wu, in
  * adapters[i] (adapterCount records) and rowAdapter (m) lie in device memory, so that a captured pass serves whichever requests are live
  * when it is replayed; they and the weights are fetched while the call before still runs, like the weights of infdev_linear: copies write them, not the
  * call before. type: INFDEV_F32,
- * INFDEV_F16 or INFDEV_BF16. Products and sums are fp32 (of fp32 operands at least 21 bits enter a product). A call gives the same bits again, and a
+ * INFDEV_F16 or INFDEV_BF16. Products and sums are fp32 (of fp32 operands at least 21 bits enter a product; beside INFDEV_F16 weights at least 21 bits
+ * or what is above 2^-39 of the largest operand taken with it: the other activations of its 32 along k, or the other inner products of its row and matrix). A call gives the same bits again, and a
  * row's are the same whatever it is taken with, as long as no more than eight rows of its 32 have its adapter; with more the order of its sums may be another. An activation that is not
  * finite makes its row's products NaN or infinite, and no other row's; weights and scale are finite. k: a multiple of 256; x lies on a 16-byte boundary, records on 8-byte ones,
  * everything else on those of its type (weights on 16-byte boundaries, a rank and n that are multiples of 8 are served fastest). n: up to 2^20; rank: up to 256; a row of a larger one

@@ -19,8 +19,8 @@
 // a quarter of 32 rows and not all of them. Weights of 16 bits are operands as they lie in memory: the order of the dimension that is summed over is
 // free, so a lane takes as many consecutive weights as one load brings, and nothing is converted or staged. What they meet, activations and inner products, is
 // cut into operands of their type: three bf16 of eight bits each, which is all of an fp32, or two fp16 of 11 bits each after a power of two that brings the
-// largest of a row's values at hand below 2^15 (what is lost of a value is below 2^-22 of it or 2^-40 of the largest). Weights of fp32 are three bf16 too; of the nine
-// products the three smallest, below 2^-24, are left out.
+// largest of a row's values at hand to 2^14 .. 2^15 (what is lost of a value is below 2^-22 of it or, where its second fp16 is subnormal, 2^-39 of the largest). Weights of fp32
+// are three bf16 too; of the nine products the three smallest are left out: pieces are cut off, not rounded, so that what is left out is below 2^-21 of the product.
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <type_traits>
