@@ -172,7 +172,7 @@ template <int ROWS, bool PAIR> __device__ __forceinline__ Block find_block(const
       rank = p.adapters[i][found.which].rank;
     if (rank > uint32_t(kAdapterMaxRank)) {
       if (report)
-        atomicExch(p.status, kStatusBadArgument);
+        atomicCAS(p.status, kStatusOk, kStatusBadArgument);  // a wait that was abandoned before, which spoils all rows, stays reported
       rank = 0;
     }
     found.rank[i] = int(rank);
