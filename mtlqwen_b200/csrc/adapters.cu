@@ -3,17 +3,18 @@
 // and for the pair of an MLP y = silu(gate + s B (A x)) * (up + s' B' (A' x)).
 //
 // The two products hang together by the r inner products of a row, which need all of k before the first of n results can be had. Two launches: the first
-// leaves the inner products of a few parts of k in a workspace, the second adds these up, multiplies and adds to the rows. The second starts early: it has its
-// weights when the first one ends.
+// leaves the inner products of a few parts of k in a workspace, the second adds these up, multiplies and adds to the rows. The second starts early where its CTAs
+// find room: in passes of up to eight rows they have their weights when the first one ends. Of more rows a CTA of the first takes all registers of its SM, and the second's come after it.
 //
 // Rows find their adapters among 32 (8, in calls of no more): the rows of one adapter are taken together, and what there is to do for all adapters of such a
-// block is dealt to its CTAs on the device, which alone knows it: the first launch by (adapter, 32 or 128 ranks of all matrices, part of k), the second by equal shares of
+// block is dealt to its CTAs on the device, which alone knows it: the first launch by (adapter, 32, 64 or 128 ranks of all matrices, part of k), the second by equal shares of
 // the columns, weighted with the ranks that stand behind them.
 //
-// What bounds it, on a B200 whose copies reach 6.46 TB/s: a single row of rank 16 (0.3 MB of weights) takes 4.0 us, of which 2.8 are two launches that do nothing; eight rows of seven
-// adapters beside three projections (12.7 MB) 9.0 us, three times the time of their bytes: each launch is a chain of row -> adapter -> rank and address -> weights and activations -> sum.
-// With many rows it is the products of the first launch and what the second fetches from shared memory for its own (of its L1 cycles, 64% are taken): 512 rows of rank 64 beside 12288 columns take
-// 35.3 us, of which the second launch has 18: 3 to add up the parts, 12 for six units of columns a warp.
+// What bounds it, on a B200 whose copies reach 6.46 TB/s: a single row of rank 16 (0.3 MB of weights) takes 4.0 us, of which 1.0 are two launches that do nothing; eight rows of six
+// adapters beside three projections (12.7 MB) 9.0 us, 4.6 times the time of their bytes: each launch is a chain of row -> adapter -> rank and address -> weights and activations -> sum,
+// and alone they take 5.6 us, of which the products 1.8, and 6.6, of which adding up, products and columns 2.2.
+// With many rows it is the products of the first launch and the rows of the second: 512 rows of rank 64 beside 12288 columns take 35.3 us; alone the first launch takes 13.6, of which the
+// products 7.2, and the second 26.5: 6.4 before its columns, 1.8 to add up the parts, 3.3 for products, 15 for the rows (50 MB, 7.8 us at the copies' rate) and weights of six units a warp.
 //
 // Both products run on the tensor cores as m16n8k16, the weights as the 16 rows of an MMA and the rows of the pass as its 8 columns, so that a single token costs
 // a quarter of 32 rows and not all of them. Weights of 16 bits are operands as they lie in memory: the order of the dimension that is summed over is
@@ -1005,7 +1006,7 @@ template <class W, bool PAIR, int NT> cudaError_t launch_blocks(const AdapterPar
   int64_t units = 0;
   for (int i = 0; i < (PAIR ? 1 : p.count); ++i)
     units += (p.n[i] + kUnit - 1) / kUnit;
-  // What there is to do only the device knows: as many CTAs as run at once, or as could have something to do.
+  // What there is to do only the device knows: two CTAs an SM, or as many as could have something to do. (In the first launch of more than eight rows one of them runs at a time.)
   const int64_t items = std::clamp<int64_t>(2 * sms / kParts / blocks, 1, most * 8);
   if (const cudaError_t e = launch_kernel<2>(inner, dim3(kParts, unsigned(blocks), unsigned(items)), inner_warps(NT) * kWarp, kInnerBytes, stream, p))
     return e;
